@@ -60,7 +60,7 @@ def listed():
         # the layer that ends a feed-forward block, on one token
         _linear("one token 4096 to 1024", BF16, False, 1, 1024, 4096, residual=True),
         # first encoder layer of a batch of cells, 5000 genes to 2048, training
-        _linear("train 512 x 5000 to 2048", F32, True, 512, 2048, 5000, act="gelu"),
+        _linear("train 512 x 5000 to 2048", F32, True, 512, 2048, 5000, act="leaky"),
         # the layer that opens a feed-forward block, on a batch's tokens, training
         _linear("train 8192 x 1024 to 4096", BF16, True, 8192, 4096, 1024, act="gelu"),
     ]
@@ -77,10 +77,8 @@ def draw(rng):
     if op == "linear":
         N, K = _log(rng, 16, 5000), _log(rng, 16, 5000)
         top = (1 << 35) // (1 if dtype == BF16 else 8)
-        # leaky has two slopes at 0: in float32 training one value of a million within its rounding of 0 takes the other
-        # slope, in the plain form as in a kernel, and stands out of 24 bits
-        acts = ["none", "gelu", "silu"] + ([] if train and dtype == F32 else ["leaky"])
-        return _linear(None, dtype, train, _log(rng, 1, max(2, min(32768, top // (N * K)))), N, K, rng.choice(acts), rng.random() < 0.5, rng.random() < 0.8)
+        return _linear(None, dtype, train, _log(rng, 1, max(2, min(32768, top // (N * K)))), N, K,
+                       rng.choice(["none", "leaky", "gelu", "silu"]), rng.random() < 0.5, rng.random() < 0.8)
     if op == "ln":
         N = _log(rng, 16, 20000)
         top = (1 << 28) // (1 if dtype == BF16 else 4)
