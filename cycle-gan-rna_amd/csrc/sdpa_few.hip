@@ -408,7 +408,8 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_bwd_kernel(AttnArgs a) {
       for (int j = 0; j < 4; ++j) s[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], sl2, ls[j]));
     }
     if (a.causal) {
-      const int from = (key0 + row - off) * a.G - 4 * half;      // rows from here on see this lane's key
+      // rows from here on see this lane's key; all of them where it is negative, which times G may pass 32 bits
+      const int from = max(key0 + row - off, 0) * a.G - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (8 * (r >> 2) + (r & 3) < from) s[r] = 0.f;

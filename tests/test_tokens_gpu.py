@@ -812,3 +812,18 @@ def test_linear_rows_far_apart(M):
     one = torch.autograd.grad(tokens.linear(a, b), (a, b), want)
     two = torch.autograd.grad(tokens.linear(c, d), (c, d), want)
     assert all(torch.equal(s, t) for s, t in zip(one, two))
+
+
+def test_few_rows_over_a_context_of_2_to_26_keys():
+    """32 query heads over one key head and 2^26 + 64 keys: rows times keys pass 2^31.  Causal order hides nothing from a
+    single query, so its gradients have the bits of the call without it."""
+    Sk, H, D = (1 << 26) + 64, 32, 8
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, do = (torch.randn(1, 1, H, D, generator=gen, device="cuda", dtype=BF) for _ in range(2))
+    k, v = (torch.randn(1, Sk, 1, D, generator=gen, device="cuda", dtype=BF) for _ in range(2))
+
+    def run(causal):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        return torch.autograd.grad(tokens.attention(*leaves, causal=causal), leaves, do)
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b) and b[:, :64].any()
