@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(64 * W, sizeof(T) == 4 && DP == 128 ? 1 : 2) a
   }
   const From from_q(W, wave, lane, (unsigned)(a.sq.s * sizeof(T)), a.D);
   const From from_g(W, wave, lane, (unsigned)(a.sdo.s * sizeof(T)), a.D);
-  // rows outside the tensor arrive as zeros, statistics too: their probabilities are 1, but do and dp are 0
+  // rows outside the tensor arrive as zeros, statistics too
   auto issue = [&](int st, int buf) {
     const int head = kvh * group + st / tq, r0 = (t0 + st % tq) * BK, left = a.Sq - r0;
     u64 rows = left >= 64 ? ~0ull : (1ull << left) - 1;
@@ -476,6 +476,14 @@ __global__ void __launch_bounds__(64 * W, sizeof(T) == 4 && DP == 128 ? 1 : 2) a
         const f32x4 ls = *reinterpret_cast<const f32x4*>(&stats[buf][0][32 * nt + 8 * g + 4 * half]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], sl2, ls[j]));
+      }
+      if (q0 < first || q0 + 32 > a.Sq) {      // rows of zeros: 0 times an infinity at a visible key is none
+        const int lo = first - q0 - 4 * half, hi = a.Sq - q0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = 8 * (r >> 2) + (r & 3);
+          if (row < lo || row >= hi) s[r] = dp[r] = 0.f;
+        }
       }
       if (q0 < free_first) {
         const int from = key - off - q0 - 4 * half;        // rows from here on see this lane's key

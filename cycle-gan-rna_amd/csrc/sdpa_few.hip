@@ -342,9 +342,10 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_bwd_kernel(AttnArgs a) {
       *reinterpret_cast<u32x4*>(qs + at) = qf[c];
       *reinterpret_cast<u32x4*>(gs + at) = gf[c];
     }
-    if (half == 0) stats[0][row] = some ? base : 0.f, stats[1][row] = nd;      // rows of zeros: p = 1, do = dp = 0
+    if (half == 0) stats[0][row] = some ? base : 0.f, stats[1][row] = nd;
   }
   __syncthreads();
+  const uint32_t taking = (uint32_t)__ballot(some);      // the rows that take part, in every wave
   const T* kb = (const T*)a.k + b * a.sk.b + kvh * a.sk.h;
   const T* vb = (const T*)a.v + b * a.sv.b + kvh * a.sv.h;
   const u64* words = a.words ? a.words + (long long)b * a.nw : nullptr;
@@ -406,6 +407,12 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_bwd_kernel(AttnArgs a) {
       const f32x4 ls = *reinterpret_cast<const f32x4*>(&stats[0][8 * g + 4 * half]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], sl2, ls[j]));
+    }
+    if (taking != ~0u) {      // rows of zeros: 0 times an infinity at a visible key is none
+      const uint32_t w = taking >> (4 * half);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (!((w >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = dp[r] = 0.f;
     }
     if (a.causal) {
       // rows from here on see this lane's key; all of them where it is negative, which times G may pass 32 bits

@@ -827,3 +827,22 @@ def test_few_rows_over_a_context_of_2_to_26_keys():
         return torch.autograd.grad(tokens.attention(*leaves, causal=causal), leaves, do)
     for a, b in zip(run(True), run(False)):
         assert torch.equal(a, b) and b[:, :64].any()
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+@pytest.mark.parametrize("Sq,Sk,D,causal", [(40, 200, 32, False), (300, 300, 64, True), (150, 200, 128, False), (2500, 300, 128, True),
+                                             (16, 200, 64, False), (1, 200, 32, False), (20, 9, 64, True)])
+def test_rows_that_do_not_exist_meet_no_infinity(dt, Sq, Sk, D, causal):
+    """A key of -inf whose scores are all -inf has no weight: its dk and dv are 0, whatever the rows of a tile that lie behind
+    the last query, or see nothing, would make of it; the other keys' are finite."""
+    gen = torch.Generator().manual_seed(22)
+    q, k, v = rand(gen, 1, Sq, 2, D, dtype=dt), rand(gen, 1, Sk, 2, D, dtype=dt), rand(gen, 1, Sk, 2, D, dtype=dt)
+    do = rand(gen, 1, Sq, 2, D, dtype=dt)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    low = torch.rand(Sk, generator=gen) < 0.5
+    low[0] = False                                           # every row that sees a key sees this one
+    k[0, low, :, 3] = -float("inf")
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    _, dk, dv = torch.autograd.grad(tokens.attention(*leaves, causal=causal), leaves, do.cuda())
+    assert torch.isfinite(dk).all() and torch.isfinite(dv).all()
+    assert not dk[:, low].any() and not dv[:, low].any() and dv[:, ~low].any()
