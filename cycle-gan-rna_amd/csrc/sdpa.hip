@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) attn_dq_kernel(At
 // wave, which halves the reads of LDS, is slower again (one wave a SIMD: 2636 us).  8 x 1000 tokens, 8 heads of 64,
 // float32: 310 us, 106 TFLOP/s.
 template <typename T, int DP, int W, bool KEYS_LDS>
-__global__ void __launch_bounds__(64 * W, sizeof(T) == 4 && DP == 128 ? 1 : 2) attn_dkv_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * W, sizeof(T) == 4 && DP == 128 ? 1 : DP == 32 ? 4 : 2) attn_dkv_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
   constexpr int BK = TL::BK, NT = BK / 32, CH = DP / El<T>::CK;
   typedef typename TL::template Source<TL::BYTES / (1024 * W)> From;
