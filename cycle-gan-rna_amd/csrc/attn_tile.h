@@ -1,6 +1,8 @@
 // What the attention kernels share: arguments, element types, LDS tiles of rows, fragments and the second product's reads.
 // The layouts are described at the top of sdpa.hip.
 #pragma once
+#include <cfloat>
+#include <climits>
 #include "lds_dma.h"
 
 namespace attn {
@@ -227,6 +229,10 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[DP / 32]) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
 }
+
+// lse2 of a row whose weights add up to 0.  It sees no key: -inf.  All the scores that it sees are -inf: NaN, but where it is
+// one of several splits, beside which the others' scores may be finite, a number below every finite lse2.
+__device__ __forceinline__ float no_weight(bool sees, int nsplit) { return sees ? (nsplit > 1 ? -FLT_MAX : NAN) : -INFINITY; }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 

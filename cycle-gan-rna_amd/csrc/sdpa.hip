@@ -2,6 +2,7 @@
 //
 //   s = scale q k^T, key j hidden from row i where its mask bit is 0 or (causal) j > i + Sk - Sq
 //   o = softmax(s) v;  lse2 = log2(sum exp(s)) kept for the backward pass
+//   a row that sees no key: o = 0, lse2 = -inf;  one with a score of +inf, or that sees scores of -inf alone: both NaN
 //   p = exp2(log2(e) s - lse2);  delta = sum_d do o;  dp = do v^T;  ds = p (dp - delta)
 //   dv = p^T do;  dq = scale ds k;  dk = scale ds^T q
 //
@@ -82,6 +83,7 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) attn
     from_v.load(to + TL::BYTES, WAVES, wave, lane, vb + (long long)t * BK * a.sv.s, nbits, TL::ALL);
   };
   tile = next(tile);
+  const int first = tile < tend ? tile * BK + __builtin_ctzll(nbits) : INT_MAX;      // the first visible key
   if (tile < tend) issue(tile, 0);
   int buf = 0;
   while (tile < tend) {
@@ -149,8 +151,10 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) attn
     buf ^= 1;
   }
   l += other_half(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float lse2 = l == 0.f ? -INFINITY : m * sl2 + __builtin_amdgcn_logf(l);
+  // No weight at all: the row sees no key, or only scores of -inf, whose quotient is not a number
+  const float none = no_weight(first <= (a.causal ? qi + off : INT_MAX - 1), a.nsplit);
+  const float inv = l == 0.f ? (none != none ? none : 0.f) : 1.f / l;
+  const float lse2 = l == 0.f ? none : m * sl2 + __builtin_amdgcn_logf(l);
   if (!live) return;
   if (l == 0.f) clear<DP>(acc);      // not multiplied by 0: a value that only other rows see may be infinite
   const long long at = ((long long)b * a.Sq + qi) * a.H + head;
@@ -198,7 +202,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[j] += __shfl_xor(s[j], o, 64);
   total = wave_sum(total);
-  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const bool lost = top == -FLT_MAX;      // keys are seen, every score is -inf
+  const float inv = lost ? NAN : total == 0.f ? 0.f : 1.f / total;
   if (side == 0 && d < a.D) {
     s *= inv;
     if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>((float*)a.out + at * a.D + d) = s;
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   }
   if (lane == 0 && a.lse2) {
     const long long h = at % a.H, bq = at / a.H;
-    a.lse2[(bq / a.Sq * a.H + h) * a.Sq + bq % a.Sq] = total == 0.f ? -INFINITY : base + __builtin_amdgcn_logf(total);
+    a.lse2[(bq / a.Sq * a.H + h) * a.Sq + bq % a.Sq] = lost ? NAN : total == 0.f ? -INFINITY : base + __builtin_amdgcn_logf(total);
   }
 }
 

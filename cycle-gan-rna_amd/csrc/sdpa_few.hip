@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_fwd_kernel(AttnArgs a) {
   auto load_v = [&](int t, uint32_t bits) { from_v.load(vs, 1, 0, lane, vb + (long long)t * 32 * a.sv.s, bits, ~0u); };
   uint32_t bits, nbits;
   int t = next(split * a.tiles_per_split + wave, bits);
+  const int first = t < end ? t * 32 + __builtin_ctz(bits) : INT_MAX;      // this wave's first visible key
   if (t < end) load_k(t, bits), load_v(t, bits);
   while (t < end) {
     lds_wait<NL>();                            // the keys are there, the values under way
@@ -133,6 +134,8 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_fwd_kernel(AttnArgs a) {
   }
   lds_wait<0>();
   l += other_half(l);
+  // a row that sees scores of -inf alone has the lowest finite maximum, one that sees no key -inf
+  if (l == 0.f && first <= (a.causal ? qi + off : INT_MAX - 1)) m = -FLT_MAX;
   if (half == 0) stat[wave][row][0] = m, stat[wave][row][1] = l;
   __syncthreads();
   // The waves' maxima and sums joined; a wave's result scaled to the common maximum and laid down, then all of them added.
@@ -147,8 +150,8 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_fwd_kernel(AttnArgs a) {
     const float lw = stat[w][row][1];
     if (lw != 0.f) total = fmaf(lw, stat[w][row][0] == base ? 1.f : __builtin_amdgcn_exp2f((stat[w][row][0] - base) * sl2), total);
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  const float mine = l == 0.f ? 0.f : (m == base ? 1.f : __builtin_amdgcn_exp2f((m - base) * sl2)) * inv;
+  const float inv = total == 0.f ? 0.f : 1.f / total, none = no_weight(top != -INFINITY, a.nsplit);
+  const float mine = l == 0.f ? (total == 0.f && none != none ? none : 0.f) : (m == base ? 1.f : __builtin_amdgcn_exp2f((m - base) * sl2)) * inv;
   if (l == 0.f) clear<DP>(acc);
   float* part = reinterpret_cast<float*>(smem);
   part_store<DP>(part + wave * 32 * DP, acc, mine, lane);
@@ -169,7 +172,7 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_fwd_kernel(AttnArgs a) {
     }
   }
   if (wave == 0 && half == 0 && live) {
-    const float lse2 = total == 0.f ? -INFINITY : top * sl2 + __builtin_amdgcn_logf(total);
+    const float lse2 = total == 0.f ? none : top * sl2 + __builtin_amdgcn_logf(total);
     if (a.nsplit > 1) a.part_lse[split * n + ((long long)b * a.Sq + qi) * a.H + head] = lse2;
     else if (a.lse2) a.lse2[((long long)b * a.H + head) * a.Sq + qi] = lse2;
   }
@@ -246,17 +249,18 @@ __global__ void __launch_bounds__(64 * ONE_WAVES, 4) attn_one_kernel(AttnArgs a)
     float mn = m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!((bits >> (u * KPW + slot)) & 1)) s[u] = -INFINITY;
-      mn = fmaxf(mn, s[u]);
+      const bool sees = (bits >> (u * KPW + slot)) & 1;
+      if (!sees) s[u] = -INFINITY;
+      mn = fmaxf(mn, sees ? fmaxf(s[u], -FLT_MAX) : s[u]);      // keys that are seen: a finite maximum at the least
     }
-    const float base = mn == -INFINITY ? 0.f : mn, f = m == base ? 1.f : __builtin_amdgcn_exp2f((m - base) * sl2);
+    const float base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f((m - base) * sl2);
     l *= f;
 #pragma unroll
     for (int j = 0; j < VE; ++j) acc[j] *= f;
     m = mn;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float p = s[u] == base ? 1.f : __builtin_amdgcn_exp2f((s[u] - base) * sl2);
+      const float p = __builtin_amdgcn_exp2f((s[u] - base) * sl2);
       float x[VE];
       widen<T>(x, v[u]);
       l += p;
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(64 * ONE_WAVES, 4) attn_one_kernel(AttnArgs a)
   float top = m;
 #pragma unroll
   for (int o = LPK; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  float base = top == -INFINITY ? 0.f : top, f = m == base ? 1.f : __builtin_amdgcn_exp2f((m - base) * sl2);
+  float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f((m - base) * sl2);
   l *= f;
 #pragma unroll
   for (int j = 0; j < VE; ++j) acc[j] *= f;
@@ -291,12 +295,13 @@ __global__ void __launch_bounds__(64 * ONE_WAVES, 4) attn_one_kernel(AttnArgs a)
   float total = 0.f, o = 0.f;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    f = stat[w][0] == base ? 1.f : __builtin_amdgcn_exp2f((stat[w][0] - base) * sl2);
+    f = __builtin_amdgcn_exp2f((stat[w][0] - base) * sl2);
     total = fmaf(f, stat[w][1], total);
     o = fmaf(f, part[w][threadIdx.x], o);
   }
-  o *= total == 0.f ? 0.f : 1.f / total;
-  const float lse2 = total == 0.f ? -INFINITY : top * sl2 + __builtin_amdgcn_logf(total);
+  const float none = no_weight(top != -INFINITY, a.nsplit);
+  o = total == 0.f ? (none != none ? none : 0.f) : o * (1.f / total);
+  const float lse2 = total == 0.f ? none : top * sl2 + __builtin_amdgcn_logf(total);
   const long long n = (long long)a.B * a.H, at = (long long)b * a.H + head, dd = threadIdx.x;
   if (dd < a.D) {
     if (a.nsplit > 1) a.part[(split * n + at) * a.D + dd] = o;

@@ -648,9 +648,11 @@ int cg_ln_bwd(void* dX, long long lddx, const void* dY, long long lddy, const vo
  *   causal != 0: key j is visible to row i only where j <= i + Sk - Sq (the last row sees every key)
  *   words (may be NULL): B rows of (Sk + 63) / 64 64-bit words, bit j % 64 of word j / 64 set where key j of the cell is
  *     visible; cg_attention_mask_words makes them from a mask of bytes (nonzero: visible; ldm: bytes between cells)
- * A row that sees no key gives 0.  Whatever K and V hold at a key that `words` hides reaches no result; at a key that
+ * A row that sees no key gives 0; one with a score of +inf or NaN, or whose visible scores are all -inf, gives NaN (the
+ * softmax's own quotient); a score of -inf beside finite ones has no weight.  Whatever K and V hold at a key that `words` hides reaches no result; at a key that
  * only `causal` hides from a row, a NaN or infinity may reach that row (0 times it).  scale > 0.
- * lse2 (B, H, Sq; may be NULL): log2 of the sum of exp(s), -inf for a row that sees nothing; cg_attention_bwd needs it.
+ * lse2 (B, H, Sq; may be NULL): log2 of the sum of exp(s), -inf for a row that sees nothing, NaN for one whose result is;
+ * cg_attention_bwd needs it.
  * workspace: cg_attention_fwd_workspace_bytes(...) bytes, 16-byte aligned (few rows and many keys: the keys are split
  * over workgroups and the partial results joined by a second launch; 0 bytes otherwise).
  */

@@ -846,3 +846,81 @@ def test_rows_that_do_not_exist_meet_no_infinity(dt, Sq, Sk, D, causal):
     _, dk, dv = torch.autograd.grad(tokens.attention(*leaves, causal=causal), leaves, do.cuda())
     assert torch.isfinite(dk).all() and torch.isfinite(dv).all()
     assert not dk[:, low].any() and not dv[:, low].any() and dv[:, ~low].any()
+
+
+# --------------------------------------------------------------------------- #
+# infinities and NaN at visible keys                                           #
+# --------------------------------------------------------------------------- #
+KINDS = [
+    # B, H, Hkv, Sq, Sk, D: one for each way the rows and keys are divided
+    (1, 1, 1, 1, 200, 32),        # one row
+    (1, 1, 1, 1, 9000, 64),       # one row, keys split
+    (1, 2, 1, 1, 200, 32),        # few rows: heads packed
+    (2, 4, 2, 16, 5000, 64),      # few rows, keys split
+    (1, 2, 2, 20, 300, 128),
+    (1, 2, 2, 40, 200, 32),       # many rows
+    (1, 1, 1, 200, 3001, 64),     # many rows, keys split
+    (1, 2, 1, 150, 700, 128),
+]
+HOLDS = ["+inf", "-inf", "all -inf", "all but one -inf", "visible -inf", "late half -inf", "nan"]
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+@pytest.mark.parametrize("holds", HOLDS)
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", KINDS)
+def test_infinite_scores(dt, holds, B, H, Hkv, Sq, Sk, D):
+    """As the definition has it, in every kernel: a row with a score of +inf or NaN, or whose visible scores are all -inf,
+    is NaN, and so are the gradients that it takes part in; a score of -inf beside finite ones has no weight; a row that
+    sees no key stays 0.  Finite rows against float64, with the bounds at the top of this file."""
+    gen = torch.Generator().manual_seed(15)
+    q, k, v, do = (rand(gen, B, s, h, D, dtype=dt) for s, h in ((Sq, H), (Sk, Hkv), (Sk, Hkv), (Sq, H)))
+    m = torch.rand(B, Sk, generator=gen) < 0.7
+    if B > 1:
+        m[1] = False                                         # a cell without keys
+    at = int(m[0].nonzero()[m[0].sum() // 2])
+    low = holds not in ("+inf", "-inf", "nan")
+    if low:                                                  # the sign of a row's score is that of the infinity
+        q[..., 3] = q[..., 3].abs() + 0.5
+    if holds in ("+inf", "-inf", "nan"):
+        k[0, at, 0, 3] = float(holds)
+    else:
+        hit = torch.zeros(Sk, dtype=torch.bool)
+        hit[:] = True
+        if holds == "all but one -inf":
+            hit[at] = False
+        elif holds == "visible -inf":
+            hit = m[0].clone()
+        elif holds == "late half -inf":
+            hit[:Sk // 2] = False
+        k[0, hit, 0, 3] = -float("inf")
+
+    G, scale = H // Hkv, D ** -0.5
+    Q, K, V, DO = (t.double().transpose(1, 2) for t in (q, k, v, do))
+    hide = ~m[:, None, :, None]
+    K, V = torch.where(hide, 0.0, K).repeat_interleave(G, 1), V.repeat_interleave(G, 1)
+    seen = m[:, None, None, :].expand(B, H, Sq, Sk)
+    s = torch.where(seen, scale * Q @ K.transpose(2, 3), -math.inf)
+    some = seen.any(-1, keepdim=True)
+    p = torch.where(seen, torch.softmax(s, -1), 0.0)
+    o = p @ V
+    dp = DO @ V.transpose(2, 3)
+    ds = torch.where(seen, p * (dp - (DO * o).sum(-1, keepdim=True)), 0.0)
+    dq, dk, dv = scale * ds @ K, scale * ds.transpose(2, 3) @ Q, p.transpose(2, 3) @ DO
+    dk, dv = (t.reshape(B, Hkv, G, Sk, D).sum(2) for t in (dk, dv))
+    finite = torch.where(torch.isfinite(K), K, 0.0)
+    es = float((D * E * scale * (Q.abs() @ finite.abs().transpose(2, 3))).max())
+    mag = float(torch.where(torch.isfinite(s), s, 0.0).abs().max())
+    ep = 4 * es + 2 ** -22 * (2 + mag) + Sk * E
+    bound = ((half_step(dt) if dt == BF else 0.0) + 2 * ep + Sk * E) * (p @ V.abs()) + half_step(dt) * o.abs() + 1e-30
+
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    got = tokens.attention(*leaves, key_mask=m.cuda())
+    grads = torch.autograd.grad(got, leaves, do.cuda())
+    got = got.detach().cpu().double().transpose(1, 2)
+    nan = torch.isnan(o)
+    assert nan.any() or holds not in ("all -inf", "visible -inf", "nan")
+    assert torch.equal(torch.isnan(got), nan)
+    assert ((got - o).abs() <= bound)[~nan].all()
+    assert not got[~some.expand_as(got)].any()
+    for what, a, b in zip(("dq", "dk", "dv"), grads, (dq, dk, dv)):
+        assert torch.equal(torch.isnan(a.cpu()), torch.isnan(b).transpose(1, 2)), what
