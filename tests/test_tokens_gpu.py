@@ -924,3 +924,65 @@ def test_infinite_scores(dt, holds, B, H, Hkv, Sq, Sk, D):
     assert not got[~some.expand_as(got)].any()
     for what, a, b in zip(("dq", "dk", "dv"), grads, (dq, dk, dv)):
         assert torch.equal(torch.isnan(a.cpu()), torch.isnan(b).transpose(1, 2)), what
+
+
+# --------------------------------------------------------------------------- #
+# activations                                                                  #
+# --------------------------------------------------------------------------- #
+def tail(a):
+    """Distribution function of the normal distribution (torch.special.ndtr takes it from 1 + erf: 2^-53 off at any size)."""
+    return 0.5 * torch.erfc(-a / math.sqrt(2))
+
+
+def act_bounds(a, act, dt):
+    """What a value of `act` at a and its slope may be off by, before they are rounded to dt.
+
+    gelu = a c, c the tail of the normal distribution or 1 minus it.  The tail is bell(a) t Q(t): in units of 2^-24 of its
+    value the fit of Q is off by 1.6, t = 1 / (1 + c |a|) by 4.5 (reciprocal 2, its argument 1, and it enters Q to a power of
+    up to 1.5), the eight steps of Q by 3, two products by 2, exp2 by 2, the corrected exponent by 1.5; with the product by a
+    15.6: 2^-20.  bf16 leaves the exponent a^2 / 2 log2(e) as it was rounded: half a^2 and three more units.  The slope is
+    c + a phi(a), each by the same share of its size.
+    silu = a g, g = 1 / (1 + exp(-a)): the exponent's rounding |a| units, 8 for exp2, sum, reciprocal and product, doubled;
+    slope g (1 + a (1 - g)), whose 1 - g is off by a unit of 1."""
+    u = 2.0 ** -24
+    if act == "gelu":
+        c = tail(a)
+        rel = 16 * u + (0.0 if dt == F32 else (a * a / 2 + 3) * u)
+        bell = torch.exp(-0.5 * a * a) / math.sqrt(2 * math.pi)
+        return rel * (a * c).abs(), rel * (c + a.abs() * bell)
+    g = torch.sigmoid(a)
+    rel = 2 * (a.abs() + 8) * u
+    return rel * (a * g).abs(), rel * (g + a.abs() * g * torch.sigmoid(-a)) + 2 * a.abs() * g * u
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_activation_values_and_slopes(act, dt):
+    """From -10 to 10, in the product's epilogue and (four rows) beside the dot product: the error is a share of the value,
+    however small that is, not of the argument."""
+    gen = torch.Generator().manual_seed(16)
+    a = torch.cat([torch.linspace(-10, 10, 20001), torch.randn(4000, generator=gen), -torch.logspace(-6, 1, 999)]).to(dt)
+    one = torch.ones(1, 1, dtype=dt, device="cuda")
+    x = a[:, None].cuda().requires_grad_()
+    y = tokens.linear(x, one, activation=act)
+    g, = torch.autograd.grad(y, x, torch.ones_like(y))
+    rows = torch.cat([tokens.linear(t.detach(), one, activation=act) for t in x[:2000:20].split(4)])
+    ad, u = a.double(), half_step(dt)
+    v, s = act_and_slope(ad, act, 0.0)
+    if act == "gelu":
+        v, s = ad * tail(ad), tail(ad) + ad * torch.exp(-0.5 * ad * ad) / math.sqrt(2 * math.pi)
+    bv, bs = act_bounds(ad, act, dt)
+    within(y[:, 0], v, bv + u * (v.abs() + bv) + 1e-37, "value")
+    within(rows[:, 0], v[:2000:20], (bv + u * (v.abs() + bv) + 1e-37)[:2000:20], "value of few rows")
+    within(g[:, 0], s, bs + u * (s.abs() + bs) + 1e-37, "slope")
+
+
+def test_activations_of_infinities():
+    for dt in (F32, BF):
+        x = torch.tensor([[float("inf")], [1e30], [-1e30], [-300.0], [300.0], [0.0]], dtype=dt, device="cuda")
+        one = torch.ones(1, 1, dtype=dt, device="cuda")
+        for act in ("gelu", "silu"):
+            y = tokens.linear(x, one, activation=act)[:, 0].cpu()
+            assert torch.equal(y[[0, 1, 4, 5]], x.cpu()[[0, 1, 4, 5], 0]) and not y[[2, 3]].any()
+        n = torch.full((6, 1), float("nan"), dtype=dt, device="cuda")
+        assert all(torch.isnan(tokens.linear(n, one, activation=act)).all() for act in ("gelu", "silu"))
