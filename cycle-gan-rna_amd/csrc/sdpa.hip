@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(64 * W, sizeof(T) == 4 && DP == 128 ? 1 : DP =
   // causal: rows from here on see any of the workgroup's / all of the wave's keys.  Rows before the first see none of
   // them, perhaps no key at all: they arrive as zeros, whatever their do holds
   const int first = a.causal ? max(0, seen0 - off) : 0;
-  const int wave_first = a.causal ? key0 - off : 0, free_first = a.causal ? key0 + 31 - off : 0;
+  const int wave_first = a.causal ? key0 - off : 0, free_first = a.causal ? max(key0 + 31 - off, first) : 0;
   const int t0 = first / BK, tq = max(0, (a.Sq + BK - 1) / BK - t0);       // tiles per query head
   const int steps = tq * group;
   // every block's steps are divided evenly: the blocks come in the order of their work, the longest first
@@ -482,19 +482,13 @@ __global__ void __launch_bounds__(64 * W, sizeof(T) == 4 && DP == 128 ? 1 : DP =
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], sl2, ls[j]));
       }
-      if (q0 < first || q0 + 32 > a.Sq) {      // rows of zeros: 0 times an infinity at a visible key is none
-        const int lo = first - q0 - 4 * half, hi = a.Sq - q0 - 4 * half;
+      if (q0 < free_first || q0 + 32 > a.Sq) {
+        // rows that see this lane's key; the others count for nothing, also where an infinite key met their zeros
+        const int from = (a.causal ? max(key - off, first) : 0) - q0 - 4 * half, to = a.Sq - q0 - 4 * half;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int row = 8 * (r >> 2) + (r & 3);
-          if (row < lo || row >= hi) s[r] = dp[r] = 0.f;
-        }
-      }
-      if (q0 < free_first) {
-        const int from = key - off - q0 - 4 * half;        // rows from here on see this lane's key
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if (8 * (r >> 2) + (r & 3) < from) s[r] = 0.f;
+          if (row < from || row >= to) s[r] = dp[r] = 0.f;
         }
       }
 #pragma unroll
