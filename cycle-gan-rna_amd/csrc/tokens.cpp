@@ -4,9 +4,11 @@
 //
 // Everything is enqueued on the current HIP stream of the tensors' device; results and scratch come from torch's caching
 // allocator.  The backward passes are first-order: autograd runs one with grad mode on only for create_graph=True, which
-// is refused instead of dropping the second-order terms silently.
+// is refused instead of dropping the second-order terms silently.  Forward-mode derivatives and traces are refused too.
 #include <torch/extension.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <cmath>
 #include "../../include/cgrna.h"
 
@@ -55,6 +57,16 @@ void same(const char* name, const Tensor& x, const Tensor& t, const char* what) 
 }
 void on_hip(const char* name, const Tensor& x) {
   TORCH_CHECK(x.is_cuda(), "cycle-gan-rna_amd runs on a HIP device only (", name, " got a tensor on ", x.device(), ")");
+}
+// What goes past these functions unseen: they hand addresses to kernels, so a tangent would be dropped without a word, and a
+// trace would hold the allocation of the result but not what fills it.
+void only_run(const char* name, std::initializer_list<Tensor> inputs) {
+  typedef c10::impl::TorchDispatchModeTLS Modes;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(), name,
+              ": cannot be traced (the trace would replay memory that nothing has written)");
+  for (const Tensor& t : inputs)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name,
+                ": no forward-mode derivatives (the tangent would be dropped silently)");
 }
 bool fits_int(int64_t n) { return n <= INT32_MAX; }
 // autograd takes an absent tensor as an absent optional, and counts the edges of those that are there
@@ -148,6 +160,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, bool causal,
                       "attention: key_mask has to be (", b, ", ", sk, ") bool, not ", m.sizes(), " ", type_of(m));
     TORCH_CHECK_VALUE(m.device() == q.device(), "attention: key_mask is on ", m.device(), ", q on ", q.device());
   }
+  only_run(name, {q, k, v});
   on_hip(name, q);
   const c10::OptionalDeviceGuard guard(q.device());
   Tensor words;
@@ -265,6 +278,7 @@ py::object layer_norm(const Tensor& x, const Maybe& weight_, const Maybe& bias_,
   if (weight.defined() && bias.defined())
     TORCH_CHECK_VALUE(weight.scalar_type() == bias.scalar_type(), "layer_norm: weight is ", type_of(weight), ", bias ", type_of(bias));
   TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "layer_norm: eps has to be a number that is not negative, not ", eps);
+  only_run(name, {x, weight, bias, residual});
   on_hip(name, x);
   const c10::OptionalDeviceGuard guard(x.device());
   if (weight.defined()) weight = weight.contiguous();
@@ -363,6 +377,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Maybe& bias_, const s
                   : activation == "silu" ? CG_ACT_SILU : -1;
   TORCH_CHECK_VALUE(act >= 0, "linear: activation has to be 'none', 'leaky', 'gelu' or 'silu', not '", activation, "'");
   TORCH_CHECK_VALUE(std::isfinite(slope), "linear: slope has to be a number, not ", slope);
+  only_run(name, {x, weight, bias, residual});
   on_hip(name, x);
   const c10::OptionalDeviceGuard guard(x.device());
   if (bias.defined()) bias = bias.contiguous();

@@ -150,3 +150,31 @@ def test_workspaces_grow_with_what_they_hold(dtype):
                 assert 0 <= f < 1 << 40 and N * 4 <= b < 1 << 40
     assert lib.cg_attention_fwd_workspace_bytes(64, 16, 16, 4096, 4096, 64, dtype) == 0       # enough rows: no splits
     assert lib.cg_attention_bwd_workspace_bytes(64, 16, 16, 4096, 4096, 64, dtype) == 64 * 16 * 4096 * 8
+
+
+def each(x):
+    """The three operators on (2, 8) values."""
+    q = x.view(1, 2, 1, 8)
+    return (lambda: tokens.attention(q, q, q), lambda: tokens.layer_norm(x), lambda: tokens.linear(x, z(3, 8)),
+            lambda: tokens.attention(z(1, 2, 1, 8), q, z(1, 2, 1, 8)), lambda: tokens.layer_norm(z(2, 8), residual=x),
+            lambda: tokens.linear(z(2, 8), z(3, 8), residual=x[:, :3]), lambda: tokens.linear(z(2, 4), z(8, 4), x[0]))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A result without its tangent would be one whose derivative is silently 0."""
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        for x in (z(2, 8), z(2, 8).requires_grad_()):
+            for call in each(fwd.make_dual(x, torch.ones(2, 8))):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+
+
+def test_traces_are_refused():
+    """A trace would hold the allocation of the result and not what fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for i in range(7):
+        with pytest.raises(RuntimeError, match="trac"):
+            torch.jit.trace(lambda x: each(x)[i](), z(2, 8))
+        with pytest.raises(RuntimeError, match="trac"):
+            make_fx(lambda x: each(x)[i]())(z(2, 8))
