@@ -18,6 +18,7 @@
 
 namespace {
 
+constexpr int LN_MAX_COLS = 1 << 30;     // columns are counted in 32 bits, up to 8192 past the last
 constexpr int LN_MAX_BLOCKS = 1024;      // workgroups of the backward pass: rows of partial column sums
 
 struct LnFwd {
@@ -487,7 +488,7 @@ bool ln_types_ok(int dtype, int wdtype) {
 }  // namespace
 
 extern "C" size_t cg_ln_bwd_workspace_bytes(int M, int N, int dtype) {
-  if (M < 0 || N < 1) return 0;
+  if (M < 0 || N < 1 || N > LN_MAX_COLS) return 0;
   return (size_t)ln_bwd_blocks(M, N, dtype == CG_BF16 ? 8 : 4) * 2 * N * sizeof(float);
 }
 
@@ -496,6 +497,7 @@ extern "C" int cg_ln_fwd(void* Y, long long ldy, void* S, long long lds, const v
                          int N, int dtype, int wdtype, void* stream) {
   if (M < 0 || N < 1 || (M > 0 && (!Y || !X)) || !ln_types_ok(dtype, wdtype) || (mean == nullptr) != (rstd == nullptr))
     return CG_ERR_BAD_ARG;
+  if (N > LN_MAX_COLS) return CG_ERR_UNSUPPORTED;
   if (M > 1 && (ldy < N || ldx < N || (S && lds < N) || (R && ldr < N))) return CG_ERR_BAD_ARG;
   if (M == 0) return CG_OK;
   hipStream_t st = (hipStream_t)stream;
@@ -516,6 +518,7 @@ extern "C" int cg_ln_bwd(void* dX, long long lddx, const void* dY, long long ldd
                          size_t workspace_bytes, void* stream) {
   if (M < 0 || N < 1 || (M > 0 && (!dY || !S || !mean || !rstd)) || !ln_types_ok(dtype, wdtype)) return CG_ERR_BAD_ARG;
   if (!dX && !dweight && !dbias) return CG_ERR_BAD_ARG;
+  if (N > LN_MAX_COLS) return CG_ERR_UNSUPPORTED;
   if (M > 1 && ((dX && lddx < N) || lddy < N || lds < N || (dS && ldds < N) || (R && ldr < N))) return CG_ERR_BAD_ARG;
   const bool cols = dweight || dbias;
   if (cols && (!workspace || workspace_bytes < cg_ln_bwd_workspace_bytes(M, N, dtype))) return CG_ERR_WORKSPACE;

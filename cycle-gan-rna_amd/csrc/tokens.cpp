@@ -196,7 +196,7 @@ LnOut ln_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, cons
   const int64_t n = x.size(-1);
   f.x = rows(x, n);
   const int64_t m = f.x.size(0);
-  TORCH_CHECK_VALUE(fits_int(m) && fits_int(n), "layer_norm: 2^31 rows or columns and more");
+  TORCH_CHECK_VALUE(fits_int(m), "layer_norm: 2^31 rows and more");
   f.y = fresh(x.sizes(), x);
   if (residual.defined()) {
     f.r = rows(residual, n);
@@ -263,6 +263,7 @@ py::object layer_norm(const Tensor& x, const Maybe& weight_, const Maybe& bias_,
   typed(name, x);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "layer_norm: a last axis of at least one element, not shape ", x.sizes());
   const int64_t n = x.size(-1);
+  TORCH_CHECK_VALUE(n <= int64_t(1) << 30, "layer_norm: up to 2^30 columns, not ", n);
   Tensor weight = tensor(weight_), bias = tensor(bias_);
   const Tensor residual = tensor(residual_);
   if (residual.defined()) {

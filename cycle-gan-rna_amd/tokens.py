@@ -46,7 +46,7 @@ def attention(q, k, v, *, causal=False, key_mask=None, scale=None):
 def layer_norm(x, weight=None, bias=None, *, residual=None, eps=1e-5):
     """LayerNorm over the last axis, optionally of a residual sum: norm(x + attn) of GAN_functions.py:35,54.
 
-    x: (..., N), any strides;  weight, bias: (N,) of x's type or float32, either may be None;  residual: like x.
+    x: (..., N), any strides, N up to 2^30;  weight, bias: (N,) of x's type or float32, either may be None;  residual: like x.
     Returns y of x's type; with a residual (y, s), where s = x + residual is the residual stream for the next layer (y and
     the gradients are those of the unrounded sum).  eps: not negative.
     """

@@ -620,7 +620,7 @@ int cg_gemm_timing_end(float* ms, int capacity);
 
 /*
  * s = x + r (r NULL: s = x);  y = (s - mean) / sqrt(var + eps) * weight + bias over the last axis (GAN_functions.py:35,
- * 54: norm(x + attn)).  M rows of N elements, leading dimensions in elements; X, R, Y, S of `dtype`, weight and bias
+ * 54: norm(x + attn)).  M rows of N elements (up to 2^30), leading dimensions in elements; X, R, Y, S of `dtype`, weight and bias
  * (either may be NULL) of `wdtype`: CG_F32, or CG_BF16 where dtype is.  S (may be NULL) receives the sum, mean and rstd
  * (float32, M values each; both or neither) what cg_ln_bwd needs.  Rows need only be aligned to their elements.  No
  * output overlaps an input (here and below).

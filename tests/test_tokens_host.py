@@ -178,3 +178,15 @@ def test_traces_are_refused():
             torch.jit.trace(lambda x: each(x)[i](), z(2, 8))
         with pytest.raises(RuntimeError, match="trac"):
             make_fx(lambda x: each(x)[i]())(z(2, 8))
+
+
+def test_rows_longer_than_2_to_30_are_refused():
+    """The kernels count columns in 32 bits and step past the last of them."""
+    lib = _lib.load_ctypes()
+    for N in ((1 << 30) + 1, (1 << 31) - 8, (1 << 31) - 1):
+        assert lib.cg_ln_fwd(P, N, None, 0, P, N, None, 0, None, None, 1e-5, None, None, 1, N, 0, 0, None) == -2
+        assert lib.cg_ln_bwd_workspace_bytes(1, N, 1) == 0
+        assert lib.cg_ln_bwd(P, N, P, N, None, 0, P, N, None, 0, None, P, P, P, P, 1, N, 1, 1, P, 1 << 50, None) == -2
+    with pytest.raises(ValueError, match="columns"):
+        tokens.layer_norm(z(1).expand((1 << 30) + 1))
+    assert lib.cg_ln_bwd_workspace_bytes(1, 1 << 30, 1) == 2 * 4 << 30
