@@ -516,8 +516,12 @@ void gemm_run(GemmArgs g, int dtype, float* part, hipStream_t st) {
 
 template <typename T>
 const T* pad_run(void* dst, const void* src, long long ld, int rows, int n, int ldd, hipStream_t st) {
-  const long long v = (long long)rows * (ldd / Vec<T>::N);
-  if (v > 0) linear_pad_kernel<T><<<(unsigned)((v + 255) / 256), 256, 0, st>>>((T*)dst, ldd, (const T*)src, ld, rows, n);
+  // a launch has fewer than 2^32 threads, one for each piece: more rows take several
+  const long long vpr = ldd / Vec<T>::N, most = (1ll << 31) / vpr;
+  for (long long r = 0; r < rows; r += most) {
+    const long long m = rows - r < most ? rows - r : most;
+    linear_pad_kernel<T><<<(unsigned)((m * vpr + 255) / 256), 256, 0, st>>>((T*)dst + r * ldd, ldd, (const T*)src + r * ld, ld, m, n);
+  }
   return (const T*)dst;
 }
 

@@ -986,3 +986,22 @@ def test_activations_of_infinities():
             assert torch.equal(y[[0, 1, 4, 5]], x.cpu()[[0, 1, 4, 5], 0]) and not y[[2, 3]].any()
         n = torch.full((6, 1), float("nan"), dtype=dt, device="cuda")
         assert all(torch.isnan(tokens.linear(n, one, activation=act)).all() for act in ("gelu", "silu"))
+
+
+def test_linear_copies_more_than_one_launch_of_rows():
+    """2^23 rows of 2049 float32 values, whose padded copy has 2^32 16-byte pieces and more: the first rows, the last and
+    some between against float64."""
+    M, N, K = 1 << 23, 8, 2049
+    gen = torch.Generator().manual_seed(21)
+    at = torch.tensor([0, 1, 2, M // 2 - 1, M // 2, M - 130, M - 129, M - 2, M - 1])
+    rows, w = rand(gen, len(at), K), rand(gen, N, K)
+    x = torch.zeros(M, K, device="cuda")
+    x[at.cuda()] = rows.cuda()
+    y = tokens.linear(x, w.cuda())
+    del x
+    ref = rows.double() @ w.double().T
+    within(y[at.cuda()], ref, (K + 4) * E * (rows.double().abs() @ w.double().abs().T) + E * ref.abs(), "y")
+    y[at.cuda()] = 0
+    assert not y.any()
+    del y
+    torch.cuda.empty_cache()
