@@ -1005,3 +1005,34 @@ def test_linear_copies_more_than_one_launch_of_rows():
     assert not y.any()
     del y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+def test_attention_gradient_along_itself(dt):
+    """<gradient, direction> against central differences of the definition in float64, along the gradient that the formulas
+    give: there the slope adds up as the bounds of the elements do, which have to stay well below it."""
+    gen = torch.Generator().manual_seed(17)
+    B, H, Hkv, Sq, Sk, D = 2, 4, 2, 40, 50, 32
+    cpu, gpu = make_qkv(gen, dt, B, H, Hkv, Sq, Sk, D, "dense")
+    do = rand(gen, B, Sq, H, D, dtype=dt)
+    m = torch.rand(B, Sk, generator=gen) < 0.7
+    refs, bounds = attention_reference(*cpu, do, True, m, 0.3)
+    leaves = [t.detach().requires_grad_() for t in gpu]
+    grads = torch.autograd.grad(tokens.attention(*leaves, causal=True, key_mask=m.cuda(), scale=0.3), leaves, do.cuda())
+
+    def value(x):
+        q, k, v = (t.transpose(1, 2) for t in x)
+        k, v = k.repeat_interleave(H // Hkv, 1), v.repeat_interleave(H // Hkv, 1)
+        seen = m[:, None, None] & torch.ones(Sq, Sk, dtype=torch.bool).tril(Sk - Sq)
+        s = torch.where(seen, 0.3 * q @ k.transpose(2, 3), torch.finfo(torch.float64).min)
+        return ((torch.softmax(s, -1) * seen.any(-1, keepdim=True) @ v).transpose(1, 2) * do.double()).sum()
+    x0 = [t.double() for t in cpu]
+    for i in range(3):
+        d = refs[i + 1] / refs[i + 1].square().mean().sqrt()
+        h = 1e-4
+        up, down = ([t + (h * s * d if j == i else 0) for j, t in enumerate(x0)] for s in (1, -1))
+        slope = float((value(up) - value(down)) / (2 * h))
+        got = float((grads[i].cpu().double() * d).sum())
+        limit = float((bounds[i + 1] * d.abs()).sum()) + 1e-4 * abs(slope)
+        assert limit <= 0.25 * slope, (i, limit, slope)
+        assert abs(got - slope) <= limit, (i, got, slope, limit)
