@@ -21,7 +21,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from cycle_gan_rna_amd import tokens  # noqa: E402
+from cycle_gan_rna_amd import _lib, tokens  # noqa: E402
 
 BF, F32 = torch.bfloat16, torch.float32
 E = 2.0 ** -24
@@ -1036,3 +1036,97 @@ def test_attention_gradient_along_itself(dt):
         limit = float((bounds[i + 1] * d.abs()).sum()) + 1e-4 * abs(slope)
         assert limit <= 0.25 * slope, (i, limit, slope)
         assert abs(got - slope) <= limit, (i, got, slope, limit)
+
+
+# --------------------------------------------------------------------------- #
+# workspaces                                                                   #
+# --------------------------------------------------------------------------- #
+def guarded(need, behind=1 << 20):
+    """`need` bytes and `behind` more that hold a pattern; the check that the pattern is whole."""
+    buf = torch.full((need + behind,), 0xA5, dtype=torch.uint8, device="cuda")
+    return buf.data_ptr() if need else None, lambda: bool((buf[need:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", [(1, 8, 2, 1, 5000, 64), (2, 4, 4, 1, 5003, 128), (2, 4, 2, 16, 5000, 64), (1, 2, 2, 200, 3001, 64),
+                                              (1, 4, 2, 2500, 300, 128), (1, 1, 1, 33, 2000, 8)])
+def test_attention_stays_inside_its_workspace(dt, B, H, Hkv, Sq, Sk, D):
+    """Through the C entry points, with exactly the bytes that they ask for: nothing behind them is written, and the results
+    are those of the public function.  With and without a mask and causal order, for which the splits differ."""
+    lib, code = _lib.load_ctypes(), 1 if dt == BF else 0
+    gen = torch.Generator().manual_seed(18)
+    _, (q, k, v) = make_qkv(gen, dt, B, H, Hkv, Sq, Sk, D, "dense")
+    do, m = rand(gen, B, Sq, H, D, dtype=dt).cuda(), (torch.rand(B, Sk, generator=gen) < 0.8).cuda()
+    words = torch.empty(B, (Sk + 63) // 64, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.cg_attention_mask_words(words.data_ptr(), m.data_ptr(), Sk, B, Sk, st) == 0
+    at = lambda t: (t.data_ptr(), *t.stride()[:3])  # noqa: E731
+    for masked in (False, True):
+        for causal in (0, 1):
+            args = (words.data_ptr() if masked else None, B, H, Hkv, Sq, Sk, D, D ** -0.5, causal, code)
+            o, lse = torch.empty_like(q), torch.empty(B, H, Sq, device="cuda")
+            need = lib.cg_attention_fwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, code)
+            ws, whole = guarded(need)
+            assert lib.cg_attention_fwd(o.data_ptr(), lse.data_ptr(), *at(q), *at(k), *at(v), *args, ws, need, st) == 0
+            assert whole()
+            dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+            need = lib.cg_attention_bwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, code)
+            ws, whole = guarded(need)
+            assert lib.cg_attention_bwd(dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *at(do), o.data_ptr(), lse.data_ptr(), *at(q),
+                                        *at(k), *at(v), *args, ws, need, st) == 0
+            assert whole()
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            want = tokens.attention(*leaves, causal=bool(causal), key_mask=m if masked else None)
+            for a, b in zip((o, dq, dk, dv), (want, *torch.autograd.grad(want, leaves, do))):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(5, 33, 41), (70, 90, 9001), (300, 1000, 1000), (129, 257, 513), (2, 77, 129), (2100, 2050, 72)])
+def test_linear_stays_inside_its_workspace(dt, M, N, K):
+    lib, code = _lib.load_ctypes(), 1 if dt == BF else 0
+    gen = torch.Generator().manual_seed(19)
+    x, w, b, dy = (rand(gen, *s, dtype=dt).cuda() for s in ((M, K), (N, K), (N,), (M, N)))
+    torch.cuda.synchronize()
+    st = torch.cuda.current_stream().cuda_stream
+    for act, name in ((0, "none"), (2, "gelu")):
+        y, z = torch.empty_like(dy), torch.empty_like(dy)
+        need = lib.cg_linear_fwd_workspace_bytes(M, N, K, code)
+        ws, whole = guarded(need)
+        assert lib.cg_linear_fwd(y.data_ptr(), N, z.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, b.data_ptr(), None, 0, M, N, K, act,
+                                 0.0, code, ws, need, st) == 0
+        assert whole()
+        dx, dw, db = (torch.empty_like(t) for t in (x, w, b))
+        need = lib.cg_linear_bwd_workspace_bytes(M, N, K, code)
+        ws, whole = guarded(need)
+        assert lib.cg_linear_bwd(dx.data_ptr(), K, dw.data_ptr(), db.data_ptr(), dy.data_ptr(), N, z.data_ptr(), N, x.data_ptr(), K,
+                                 w.data_ptr(), K, M, N, K, act, 0.0, code, ws, need, st) == 0
+        assert whole()
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        want = tokens.linear(*leaves, activation=name)
+        for a, c in zip((y, dx, dw, db), (want, *torch.autograd.grad(want, leaves, dy))):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+@pytest.mark.parametrize("M,N", [(3, 7), (5000, 72), (1100, 2049), (300, 12289), (70, 32769)])
+def test_layer_norm_stays_inside_its_workspace(dt, M, N):
+    lib, code = _lib.load_ctypes(), 1 if dt == BF else 0
+    gen = torch.Generator().manual_seed(20)
+    x, w, b, dy = (rand(gen, *s, dtype=dt).cuda() for s in ((M, N), (N,), (N,), (M, N)))
+    y, dx, dw, db = (torch.empty_like(t) for t in (x, x, w, b))
+    mean, rstd = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    torch.cuda.synchronize()
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.cg_ln_fwd(y.data_ptr(), N, None, 0, x.data_ptr(), N, None, 0, w.data_ptr(), b.data_ptr(), 1e-5, mean.data_ptr(),
+                         rstd.data_ptr(), M, N, code, code, st) == 0
+    need = lib.cg_ln_bwd_workspace_bytes(M, N, code)
+    ws, whole = guarded(need)
+    assert lib.cg_ln_bwd(dx.data_ptr(), N, dy.data_ptr(), N, None, 0, x.data_ptr(), N, None, 0, w.data_ptr(), mean.data_ptr(),
+                         rstd.data_ptr(), dw.data_ptr(), db.data_ptr(), M, N, code, code, ws, need, st) == 0
+    assert whole()
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    want = tokens.layer_norm(*leaves)
+    for a, c in zip((y, dx, dw, db), (want, *torch.autograd.grad(want, leaves, dy))):
+        assert torch.equal(a, c)

@@ -190,3 +190,26 @@ def test_rows_longer_than_2_to_30_are_refused():
     with pytest.raises(ValueError, match="columns"):
         tokens.layer_norm(z(1).expand((1 << 30) + 1))
     assert lib.cg_ln_bwd_workspace_bytes(1, 1 << 30, 1) == 2 * 4 << 30
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_workspaces_hold_what_goes_through_them(dtype):
+    """Lower bounds from what a call lays down: padded copies of rows that are not whole 16-byte pieces, the activation's
+    gradient and column sums of the dense layer; two partial results at least where attention's keys are split, and two
+    float32 values a row of its backward pass."""
+    lib, e, size = _lib.load_ctypes(), (4, 8)[dtype], (4, 2)[dtype]
+    up = lambda n: -(-n // e) * e  # noqa: E731
+    for M in (5, 64, 513, 8192):
+        for N in (1, 7, 64, 1000):
+            for K in (1, 33, 4096):
+                assert lib.cg_linear_fwd_workspace_bytes(M, N, K, dtype) >= (M + N) * up(K) * size
+                assert lib.cg_linear_bwd_workspace_bytes(M, N, K, dtype) >= ((M + N) * up(K) + M * up(N)) * size + 4 * N
+    split = 0
+    for B, H, Hkv, Sq, Sk, D in ((1, 8, 2, 1, 5000, 64), (2, 4, 4, 16, 5000, 64), (1, 2, 2, 200, 3001, 64), (1, 4, 2, 2500, 300, 128),
+                                 (64, 16, 16, 512, 512, 32), (1, 1, 1, 1, 1, 8)):
+        f = lib.cg_attention_fwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, dtype)
+        assert f == 0 or f >= 2 * B * Sq * H * (D + 1) * 4
+        b = lib.cg_attention_bwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, dtype)
+        assert b >= B * H * Sq * 8
+        split += (f > 0) + (b > B * H * Sq * 8 + 16)
+    assert split >= 5
