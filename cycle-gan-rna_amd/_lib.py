@@ -111,8 +111,10 @@ SIGNATURES = {
     "cg_attention_mask_words": ([P, P, L, I, I, P], I),
     "cg_attention_fwd_workspace_bytes": ([I, I, I, I, I, I, I], Z),
     "cg_attention_fwd": ([P, P] + [P, L, L, L] * 3 + [P, I, I, I, I, I, I, F, I, I, P, Z, P], I),
+    "cg_attention_fwd_low": ([P, P, P] + [P, L, L, L] * 3 + [P, I, I, I, I, I, I, F, I, I, P, Z, P], I),
     "cg_attention_bwd_workspace_bytes": ([I, I, I, I, I, I, I], Z),
     "cg_attention_bwd": ([P, P, P, P, L, L, L, P, P] + [P, L, L, L] * 3 + [P, I, I, I, I, I, I, F, I, I, P, Z, P], I),
+    "cg_attention_bwd_low": ([P, P, P, P, L, L, L, P, P, P] + [P, L, L, L] * 3 + [P, I, I, I, I, I, I, F, I, I, P, Z, P], I),
     "cg_linear_fwd_workspace_bytes": ([I, I, I, I], Z),
     "cg_linear_fwd": ([P, L, P, L, P, L, P, L, P, P, L, I, I, I, I, F, I, P, Z, P], I),
     "cg_linear_bwd_workspace_bytes": ([I, I, I, I], Z),

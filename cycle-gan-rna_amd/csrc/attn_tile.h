@@ -21,6 +21,8 @@ struct AttnArgs {
   const void *q, *k, *v, *o, *dout;
   Strides sq, sk, sv, sdo;
   void *out, *dq, *dk, *dv;                  // dense (B, S, heads, D)
+  const void* low;                           // bf16, backward: what rounding left of o (NULL: not kept)
+  void* out_low;                             // forward: where to keep it
   float *lse2, *nlse, *ndelta;               // (B, H, Sq); nlse: what the backward pass adds to log2(e) s; ndelta: -sum_d do o
   const u64* words;                          // (B, nw) mask bits, 64 keys a word; NULL: every key is visible
   float* part;                               // partial results of splits
@@ -59,6 +61,27 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack2(float a, float b) {      // one instruction: v_cvt_pk_bf16_f32
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// Four results as they are stored, to `at`, and (bf16, low not NULL) what their rounding left, to `low`: with it the backward
+// pass forms delta from 16 bits of each result, not 8.  Where a result is infinite nothing is left.
+template <typename T>
+__device__ __forceinline__ void put4(T* at, u16* low, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4*>(at) = f32x4{x[0], x[1], x[2], x[3]};
+  } else {
+    const u32x2 w = {pack2(x[0], x[1]), pack2(x[2], x[3])};
+    *reinterpret_cast<u32x2*>(at) = w;
+    if (low) {
+      float rest[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        rest[j] = x[j] - __builtin_bit_cast(float, j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+        rest[j] = fabsf(rest[j]) <= FLT_MAX ? rest[j] : 0.f;
+      }
+      *reinterpret_cast<u32x2*>(low) = u32x2{pack2(rest[0], rest[1]), pack2(rest[2], rest[3])};
+    }
+  }
 }
 
 // ---- LDS tile of `El<T>::BK` rows ----------------------------------------------------------------------------------
@@ -171,7 +194,7 @@ __device__ __forceinline__ void load_rows(u32x4 (&f)[DP / El<T>::CK], const T* p
 
 // Store a lane's row of an accumulator set: columns 32 dt + 8 g + 4 h + 0..3.
 template <typename T, int DP>
-__device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[DP / 32], float mul, int D, int lane) {
+__device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[DP / 32], float mul, int D, int lane, u16* low = nullptr) {
   const int h = lane >> 5;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
@@ -179,17 +202,10 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[DP / 32],
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * dt + 8 * g + 4 * h;
       if (d >= D) continue;
-      if constexpr (sizeof(T) == 4) {
-        f32x4 w;
+      float w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = acc[dt][4 * g + j] * mul;
-        *reinterpret_cast<f32x4*>(row + d) = w;
-      } else {
-        u32x2 w;
-        w[0] = pack2(acc[dt][4 * g] * mul, acc[dt][4 * g + 1] * mul);
-        w[1] = pack2(acc[dt][4 * g + 2] * mul, acc[dt][4 * g + 3] * mul);
-        *reinterpret_cast<u32x2*>(row + d) = w;
-      }
+      for (int j = 0; j < 4; ++j) w[j] = acc[dt][4 * g + j] * mul;
+      put4<T>(row + d, low ? low + d : nullptr, w);
     }
 }
 

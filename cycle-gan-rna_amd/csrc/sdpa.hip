@@ -13,7 +13,10 @@
 // dimension is taken in that order.  So probabilities never leave the registers, a row's maximum and sum are
 // reductions inside a lane plus one exchange between its halves, and the other operand is read from LDS in the same order
 // (bf16: ds_read_b64_tr_b16, float32: ds_read_b32).
-// bf16: p and ds are rounded to bf16 for the second product (2^-8 of each term); everything else is float32.
+// bf16: p and ds are rounded to bf16 for the second product (2^-8 of each term), since the matrix cores take nothing wider at
+// their rate; everything else is float32.  delta is formed from o as it was stored and what that rounding left (another bf16
+// value of each, kept for the backward pass alone; 2 bytes written and read per element, 0.3-1 % of a training call): from the
+// stored o alone the root mean square error of dq was 4.8-6 thousandths where one key has most of a row's weight, now 2.5-3.
 //
 // LDS tiles hold rows of DP elements (the head dimension padded to 32, 64 or 128) in 16-byte pieces, written by the
 // LDS-DMA loads lane by lane; piece p of row r sits at slot p ^ swizzle(r), so that both a column of 16 rows
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) attn
     store_rows<float, DP>(a.part + (split * n + at) * a.D, acc, inv, a.D, lane);
     if (half == 0) a.part_lse[split * n + at] = lse2;
   } else {
-    store_rows<T, DP>((T*)a.out + at * a.D, acc, inv, a.D, lane);
+    store_rows<T, DP>((T*)a.out + at * a.D, acc, inv, a.D, lane, a.out_low ? (u16*)a.out_low + at * a.D : nullptr);
     if (half == 0 && a.lse2) a.lse2[((long long)b * a.H + head) * a.Sq + qi] = lse2;
   }
 }
@@ -206,8 +209,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   const float inv = lost ? NAN : total == 0.f ? 0.f : 1.f / total;
   if (side == 0 && d < a.D) {
     s *= inv;
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>((float*)a.out + at * a.D + d) = s;
-    else *reinterpret_cast<u32x2*>((u16*)a.out + at * a.D + d) = u32x2{pack2(s[0], s[1]), pack2(s[2], s[3])};
+    const float w[4] = {s[0], s[1], s[2], s[3]};
+    put4<T>((T*)a.out + at * a.D + d, a.out_low ? (u16*)a.out_low + at * a.D + d : nullptr, w);
   }
   if (lane == 0 && a.lse2) {
     const long long h = at % a.H, bq = at / a.H;
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(256) attn_words_kernel(u64* words, const uint8
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// ndelta (B, H, Sq) = -sum_d do o, from which the products dp = do v^T start, and nlse = -lse2, or -inf for a row that sees nothing: its probabilities are all 0.
+// ndelta (B, H, Sq) = -sum_d do o (o with what its rounding to bf16 left, where that was kept), from which the products dp = do v^T start, and nlse = -lse2, or -inf for a row that sees nothing: its probabilities are all 0.
 // Eight lanes per row.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
@@ -235,19 +238,23 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
   if (at >= n) return;
   const long long h = at % a.H, bq = at / a.H, b = bq / a.Sq, q = bq % a.Sq;
   const T* o = (const T*)a.o + at * a.D;
+  const T* low = a.low ? (const T*)a.low + at * a.D : nullptr;
   const T* g = (const T*)a.dout + b * a.sdo.b + q * a.sdo.s + h * a.sdo.h;
   constexpr int E = 16 / sizeof(T);
   float s = 0.f;
   for (int d = (threadIdx.x & 7) * E; d < a.D; d += 8 * E) {
     typedef typename El<T>::Vec4 V4;
     const V4 x = *reinterpret_cast<const V4*>(o + d), y = *reinterpret_cast<const V4*>(g + d);
+    V4 z{};
+    if (sizeof(T) == 2 && low) z = *reinterpret_cast<const V4*>(low + d);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (sizeof(T) == 4) {
         s = fmaf(x[j], y[j], s);
       } else {
-        s = fmaf(__builtin_bit_cast(float, x[j] << 16), __builtin_bit_cast(float, y[j] << 16), s);
-        s = fmaf(__builtin_bit_cast(float, x[j] & 0xffff0000u), __builtin_bit_cast(float, y[j] & 0xffff0000u), s);
+        const float y0 = __builtin_bit_cast(float, y[j] << 16), y1 = __builtin_bit_cast(float, y[j] & 0xffff0000u);
+        s = fmaf(__builtin_bit_cast(float, x[j] << 16) + __builtin_bit_cast(float, z[j] << 16), y0, s);
+        s = fmaf(__builtin_bit_cast(float, x[j] & 0xffff0000u) + __builtin_bit_cast(float, z[j] & 0xffff0000u), y1, s);
       }
     }
   }
@@ -697,21 +704,30 @@ extern "C" int cg_attention_fwd(void* O, float* lse2, const void* Q, long long q
                                 long long kb, long long ks, long long kh, const void* V, long long vb, long long vs,
                                 long long vh, const void* words, int B, int H, int Hkv, int Sq, int Sk, int D, float scale,
                                 int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return cg_attention_fwd_low(O, nullptr, lse2, Q, qb, qs, qh, K, kb, ks, kh, V, vb, vs, vh, words, B, H, Hkv, Sq, Sk, D, scale,
+                              causal, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int cg_attention_fwd_low(void* O, void* Olow, float* lse2, const void* Q, long long qb, long long qs, long long qh, const void* K,
+                                long long kb, long long ks, long long kh, const void* V, long long vb, long long vs,
+                                long long vh, const void* words, int B, int H, int Hkv, int Sq, int Sk, int D, float scale,
+                                int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   const int ok = attn_shape_ok(B, H, Hkv, Sq, Sk, D, dtype);
   if (ok != CG_OK) return ok;
   if (!(scale > 0.f) || scale > 3e38f) return CG_ERR_BAD_ARG;
   if (B == 0 || Sq == 0) return CG_OK;
-  if (!O || !Q || (Sk > 0 && (!K || !V))) return CG_ERR_BAD_ARG;
+  if (!O || !Q || (Sk > 0 && (!K || !V)) || (Olow && dtype != CG_BF16)) return CG_ERR_BAD_ARG;
   const Strides sq{qb, qs, qh}, sk{kb, ks, kh}, sv{vb, vs, vh};
   if (!operand_ok(Q, sq, B, Sq, H, dtype) || !operand_ok(K, sk, B, Sk, Hkv, dtype) || !operand_ok(V, sv, B, Sk, Hkv, dtype) ||
-      ((uintptr_t)O & 15))
+      (((uintptr_t)O | (uintptr_t)Olow) & 15))
     return CG_ERR_UNSUPPORTED;
   const Plan p = row_plan(B, H, Hkv, Sq, Sk, D, dtype, false, words != nullptr);
   if (p.nsplit > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
                        workspace_bytes < cg_attention_fwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, dtype)))
     return CG_ERR_WORKSPACE;
   AttnArgs a{};
-  a.q = Q, a.k = K, a.v = V, a.sq = sq, a.sk = sk, a.sv = sv, a.out = O, a.lse2 = lse2, a.words = (const u64*)words;
+  a.q = Q, a.k = K, a.v = V, a.sq = sq, a.sk = sk, a.sv = sv, a.out = O, a.out_low = Olow, a.lse2 = lse2;
+  a.words = (const u64*)words;
   a.B = B, a.H = H, a.Hkv = Hkv, a.Sq = Sq, a.Sk = Sk, a.D = D, a.nw = (Sk + 63) / 64, a.scale = scale, a.causal = causal;
   a.part = (float*)workspace;
   if (p.nsplit > 1) a.part_lse = (float*)((char*)workspace + up16((size_t)B * Sq * H * p.nsplit * D * 4));
@@ -739,20 +755,30 @@ extern "C" int cg_attention_bwd(void* dQ, void* dK, void* dV, const void* dO, lo
                                 const void* K, long long kb, long long ks, long long kh, const void* V, long long vb,
                                 long long vs, long long vh, const void* words, int B, int H, int Hkv, int Sq, int Sk, int D,
                                 float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return cg_attention_bwd_low(dQ, dK, dV, dO, gb, gs, gh, O, nullptr, lse2, Q, qb, qs, qh, K, kb, ks, kh, V, vb, vs, vh, words, B, H,
+                              Hkv, Sq, Sk, D, scale, causal, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int cg_attention_bwd_low(void* dQ, void* dK, void* dV, const void* dO, long long gb, long long gs, long long gh,
+                                const void* O, const void* Olow, const float* lse2, const void* Q, long long qb, long long qs, long long qh,
+                                const void* K, long long kb, long long ks, long long kh, const void* V, long long vb,
+                                long long vs, long long vh, const void* words, int B, int H, int Hkv, int Sq, int Sk, int D,
+                                float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   const int ok = attn_shape_ok(B, H, Hkv, Sq, Sk, D, dtype);
   if (ok != CG_OK) return ok;
   if (!(scale > 0.f) || scale > 3e38f) return CG_ERR_BAD_ARG;
   if (B == 0 || (Sq == 0 && Sk == 0)) return CG_OK;
-  if ((Sq > 0 && (!dQ || !dO || !O || !lse2 || !Q)) || (Sk > 0 && (!dK || !dV || !K || !V))) return CG_ERR_BAD_ARG;
+  if ((Sq > 0 && (!dQ || !dO || !O || !lse2 || !Q)) || (Sk > 0 && (!dK || !dV || !K || !V)) || (Olow && dtype != CG_BF16))
+    return CG_ERR_BAD_ARG;
   const Strides sq{qb, qs, qh}, sk{kb, ks, kh}, sv{vb, vs, vh}, sg{gb, gs, gh};
   if (!operand_ok(Q, sq, B, Sq, H, dtype) || !operand_ok(K, sk, B, Sk, Hkv, dtype) || !operand_ok(V, sv, B, Sk, Hkv, dtype) ||
-      !operand_ok(dO, sg, B, Sq, H, dtype) || (((uintptr_t)O | (uintptr_t)dQ | (uintptr_t)dK | (uintptr_t)dV) & 15))
+      !operand_ok(dO, sg, B, Sq, H, dtype) || (((uintptr_t)O | (uintptr_t)Olow | (uintptr_t)dQ | (uintptr_t)dK | (uintptr_t)dV) & 15))
     return CG_ERR_UNSUPPORTED;
   if (workspace_bytes < cg_attention_bwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, dtype) || ((uintptr_t)workspace & 15) ||
       (Sq > 0 && !workspace))
     return CG_ERR_WORKSPACE;
   AttnArgs a{};
-  a.q = Q, a.k = K, a.v = V, a.o = O, a.dout = dO, a.sq = sq, a.sk = sk, a.sv = sv, a.sdo = sg;
+  a.q = Q, a.k = K, a.v = V, a.o = O, a.low = Olow, a.dout = dO, a.sq = sq, a.sk = sk, a.sv = sv, a.sdo = sg;
   a.dq = dQ, a.dk = dK, a.dv = dV, a.lse2 = const_cast<float*>(lse2), a.words = (const u64*)words;
   a.B = B, a.H = H, a.Hkv = Hkv, a.Sq = Sq, a.Sk = Sk, a.D = D, a.nw = (Sk + 63) / 64, a.scale = scale, a.causal = causal;
   a.nlse = (float*)workspace, a.ndelta = a.nlse + (size_t)B * H * Sq;

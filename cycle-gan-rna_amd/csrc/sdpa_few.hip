@@ -165,10 +165,9 @@ __global__ void __launch_bounds__(64 * W, 1) attn_few_fwd_kernel(AttnArgs a) {
     const long long at = ((long long)b * a.Sq + r / a.G) * a.H + hu * a.G + r % a.G;
     if (a.nsplit > 1) {
       *reinterpret_cast<f32x4*>(a.part + (split * n + at) * a.D + d) = o;
-    } else if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<f32x4*>((float*)a.out + at * a.D + d) = o;
     } else {
-      *reinterpret_cast<u32x2*>((u16*)a.out + at * a.D + d) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+      const float x[4] = {o[0], o[1], o[2], o[3]};
+      put4<T>((T*)a.out + at * a.D + d, a.out_low ? (u16*)a.out_low + at * a.D + d : nullptr, x);
     }
   }
   if (wave == 0 && half == 0 && live) {
@@ -306,7 +305,12 @@ __global__ void __launch_bounds__(64 * ONE_WAVES, 4) attn_one_kernel(AttnArgs a)
   if (dd < a.D) {
     if (a.nsplit > 1) a.part[(split * n + at) * a.D + dd] = o;
     else if constexpr (sizeof(T) == 4) ((float*)a.out)[at * a.D + dd] = o;
-    else ((u16*)a.out)[at * a.D + dd] = f2bf(o);
+    else {
+      const u16 w = f2bf(o);
+      ((u16*)a.out)[at * a.D + dd] = w;
+      const float rest = o - bf2f(w);
+      if (a.out_low) ((u16*)a.out_low)[at * a.D + dd] = f2bf(fabsf(rest) <= FLT_MAX ? rest : 0.f);
+    }
   }
   if (dd == 0) {
     if (a.nsplit > 1) a.part_lse[split * n + at] = lse2;

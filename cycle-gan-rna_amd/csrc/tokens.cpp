@@ -98,15 +98,20 @@ struct AttnShape {
       : B(q.size(0)), H(q.size(2)), Hkv(k.size(2)), Sq(q.size(1)), Sk(k.size(1)), D(q.size(3)), dt(code_of(q)) {}
 };
 
+// For the backward pass: log2 of the sum of exp(s), and in bf16 what the rounding of o left (delta = sum_d do o is formed from both)
+struct Kept { Tensor lse2, low; };
+
 Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& words, double scale, bool causal,
-                         Tensor* lse2) {
+                         Kept* keep) {
   const AttnShape s(q, k);
   Tensor o = fresh(q.sizes(), q);
-  if (lse2) *lse2 = floats({s.B, s.H, s.Sq}, q);
+  if (keep) keep->lse2 = floats({s.B, s.H, s.Sq}, q);
+  if (keep && s.dt == CG_BF16) keep->low = fresh(q.sizes(), q);
   const Tensor ws = bytes(cg_attention_fwd_workspace_bytes(s.B, s.H, s.Hkv, s.Sq, s.Sk, s.D, s.dt), q);
-  check(cg_attention_fwd(ptr(o), lse2 ? (float*)ptr(*lse2) : nullptr, STRIDED(q), STRIDED(k), STRIDED(v), ptr(words), s.B, s.H,
-                         s.Hkv, s.Sq, s.Sk, s.D, (float)scale, causal, s.dt, ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(q)),
-        "cg_attention_fwd");
+  check(cg_attention_fwd_low(ptr(o), keep ? ptr(keep->low) : nullptr, keep ? (float*)ptr(keep->lse2) : nullptr, STRIDED(q),
+                             STRIDED(k), STRIDED(v), ptr(words), s.B, s.H, s.Hkv, s.Sq, s.Sk, s.D, (float)scale, causal, s.dt,
+                             ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(q)),
+        "cg_attention_fwd_low");
   return o;
 }
 
@@ -114,9 +119,9 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const Maybe& words_,
                         double scale, bool causal) {
     const Tensor words = tensor(words_), q = pieces(q0), k = pieces(k0), v = pieces(v0);
-    Tensor lse2;
-    Tensor o = attention_forward(q, k, v, words, scale, causal, &lse2);
-    ctx->save_for_backward({q, k, v, o, lse2, words});
+    Kept keep;
+    Tensor o = attention_forward(q, k, v, words, scale, causal, &keep);
+    ctx->save_for_backward({q, k, v, o, keep.low, keep.lse2, words});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     return o;
@@ -124,16 +129,17 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     first_order_only();
     const auto saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse2 = saved[4], &words = saved[5];
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &low = saved[4], &lse2 = saved[5], &words = saved[6];
     const c10::OptionalDeviceGuard guard(q.device());
     const Tensor g = pieces(grads[0]);
     const AttnShape s(q, k);
     Tensor dq = fresh(q.sizes(), q), dk = fresh(k.sizes(), q), dv = fresh(k.sizes(), q);
     const Tensor ws = bytes(cg_attention_bwd_workspace_bytes(s.B, s.H, s.Hkv, s.Sq, s.Sk, s.D, s.dt), q);
-    check(cg_attention_bwd(ptr(dq), ptr(dk), ptr(dv), STRIDED(g), ptr(o), (const float*)ptr(lse2), STRIDED(q), STRIDED(k),
-                           STRIDED(v), ptr(words), s.B, s.H, s.Hkv, s.Sq, s.Sk, s.D, (float)ctx->saved_data["scale"].toDouble(),
-                           ctx->saved_data["causal"].toBool(), s.dt, ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(q)),
-          "cg_attention_bwd");
+    check(cg_attention_bwd_low(ptr(dq), ptr(dk), ptr(dv), STRIDED(g), ptr(o), ptr(low), (const float*)ptr(lse2), STRIDED(q),
+                               STRIDED(k), STRIDED(v), ptr(words), s.B, s.H, s.Hkv, s.Sq, s.Sk, s.D,
+                               (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(), s.dt, ptr(ws),
+                               ws.defined() ? ws.numel() : 0, stream_of(q)),
+          "cg_attention_bwd_low");
     return {dq, dk, dv, Tensor(), Tensor(), Tensor()};
   }
 };

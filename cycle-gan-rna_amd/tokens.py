@@ -37,7 +37,8 @@ def attention(q, k, v, *, causal=False, key_mask=None, scale=None):
         rows, a NaN or infinity may reach those rows.)
     scale: a positive number, default D ** -0.5.
     Returns (B, Sq, H, D) of q's type.  A row that sees no key gives 0, and 0 gradient to q.  A row with a score of +inf or
-    NaN, or whose visible scores are all -inf, gives NaN, and NaN to the gradients that it takes part in.  One query (Sq = 1) or few
+    NaN, or whose visible scores are all -inf, gives NaN, and NaN to the gradients that it takes part in.  bfloat16: the
+    probabilities and the scores' gradients are rounded to bfloat16 for the products with v, q, k and the output's gradient.  One query (Sq = 1) or few
     rows over many keys are split over the keys.  Lengths of 0 are allowed.
     """
     return _lib.load_tokens().attention(q, k, v, causal, key_mask, scale)

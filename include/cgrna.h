@@ -662,11 +662,19 @@ int cg_attention_fwd(void* O, float* lse2, const void* Q, long long qb, long lon
                      long long kb, long long ks, long long kh, const void* V, long long vb, long long vs, long long vh,
                      const void* words, int B, int H, int Hkv, int Sq, int Sk, int D, float scale, int causal, int dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
+/* The same, and in Olow (CG_BF16, dense like O; NULL: not wanted) what the rounding of O to bf16 left, itself in bf16. */
+int cg_attention_fwd_low(void* O, void* Olow, float* lse2, const void* Q, long long qb, long long qs, long long qh,
+                         const void* K, long long kb, long long ks, long long kh, const void* V, long long vb, long long vs,
+                         long long vh, const void* words, int B, int H, int Hkv, int Sq, int Sk, int D, float scale,
+                         int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 /*
  * Its gradient, with the probabilities recomputed from lse2 (no Sq x Sk matrix is kept or written):
  *   p = exp(s - lse), delta = sum_d do o;  dv = p^T do;  ds = p (do v^T - delta);  dq = scale ds k;  dk = scale ds^T q
  * dQ, dK, dV dense like O, K and V; the gradients of a key head are summed over its query heads.  dO with strides like Q.
  * Sums in a fixed order, no atomics: the same bits every time.  A masked key's dk and dv are 0, an unseeing row's dq.
+ * CG_BF16: p and ds are rounded to bf16 for the second products (2^-8 of each term), and so is o for delta, unless
+ * cg_attention_bwd_low gets what that rounding left: where one key has most of a row's weight, dp - delta is a small
+ * difference, and the gradients are then half as far off.
  */
 size_t cg_attention_bwd_workspace_bytes(int B, int H, int Hkv, int Sq, int Sk, int D, int dtype);
 int cg_attention_bwd(void* dQ, void* dK, void* dV, const void* dO, long long gb, long long gs, long long gh, const void* O,
@@ -674,6 +682,11 @@ int cg_attention_bwd(void* dQ, void* dK, void* dV, const void* dO, long long gb,
                      long long kb, long long ks, long long kh, const void* V, long long vb, long long vs, long long vh,
                      const void* words, int B, int H, int Hkv, int Sq, int Sk, int D, float scale, int causal, int dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
+int cg_attention_bwd_low(void* dQ, void* dK, void* dV, const void* dO, long long gb, long long gs, long long gh,
+                         const void* O, const void* Olow, const float* lse2, const void* Q, long long qb, long long qs,
+                         long long qh, const void* K, long long kb, long long ks, long long kh, const void* V, long long vb,
+                         long long vs, long long vh, const void* words, int B, int H, int Hkv, int Sq, int Sk, int D,
+                         float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Dense layer with everything that follows the product in its epilogue (nn.Linear and the activation after it,
