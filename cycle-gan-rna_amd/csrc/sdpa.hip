@@ -16,7 +16,8 @@
 // bf16: p and ds are rounded to bf16 for the second product (2^-8 of each term), since the matrix cores take nothing wider at
 // their rate; everything else is float32.  delta is formed from o as it was stored and what that rounding left (another bf16
 // value of each, kept for the backward pass alone; 2 bytes written and read per element, 0.3-1 % of a training call): from the
-// stored o alone the root mean square error of dq was 4.8-6 thousandths where one key has most of a row's weight, now 2.5-3.
+// stored o alone the root mean square error of dq was 3.6-6.0 thousandths of dq where one key has most of a row's weight, with
+// what rounding left 2.1-3.4 (2.1: dq's own rounding).
 //
 // LDS tiles hold rows of DP elements (the head dimension padded to 32, 64 or 128) in 16-byte pieces, written by the
 // LDS-DMA loads lane by lane; piece p of row r sits at slot p ^ swizzle(r), so that both a column of 16 rows

@@ -38,8 +38,8 @@ def attention(q, k, v, *, causal=False, key_mask=None, scale=None):
     scale: a positive number, default D ** -0.5.
     Returns (B, Sq, H, D) of q's type.  A row that sees no key gives 0, and 0 gradient to q.  A row with a score of +inf or
     NaN, or whose visible scores are all -inf, gives NaN, and NaN to the gradients that it takes part in.  bfloat16: the
-    probabilities and the scores' gradients are rounded to bfloat16 for the products with v, q, k and the output's gradient.  One query (Sq = 1) or few
-    rows over many keys are split over the keys.  Lengths of 0 are allowed.
+    probabilities and the scores' gradients are rounded to bfloat16 for the products with v, q, k and the output's
+    gradient.  One query (Sq = 1) or few rows over many keys are split over the keys.  Lengths of 0 are allowed.
     """
     return _lib.load_tokens().attention(q, k, v, causal, key_mask, scale)
 
@@ -61,7 +61,9 @@ def linear(x, weight, bias=None, *, activation="none", slope=0.0, residual=None)
     activation: "none", "leaky" (values a <= 0 times `slope`; 0 is ReLU), "gelu" (a times the normal distribution
         function at a) or "silu" (a / (1 + exp(-a))).
     Returns (..., N).  Products are exact float32 or bf16 with float32 sums; bias, activation and residual are applied in
-    float32 and the result is rounded once.  Rows of K (and for the backward pass N) that are not whole 16-byte
-    pieces cost a padded copy.
+    float32 and the result is rounded once.  For the backward pass bfloat16 keeps a = x weight^T + bias as rounded to
+    bfloat16, and the gradient of a is rounded to bfloat16 for its products with x and weight (the bias's is summed
+    before).  Values of gelu are right to a share of themselves however small they are (float32: 2^-20).  Rows of K (and
+    for the backward pass N) that are not whole 16-byte pieces cost a padded copy.
     """
     return _lib.load_tokens().linear(x, weight, bias, activation, slope, residual)
