@@ -12,10 +12,10 @@ storage.
 
 Tensors are float32 or bfloat16 on a HIP device; sums, statistics and the softmax are float32 in either case.  Calls are
 enqueued on the device's current stream, allocate through torch's caching allocator (so they can be captured into a HIP
-graph after one eager call) and have first-order gradients; forward-mode derivatives and tracing raise RuntimeError.  There is no CPU or eager-PyTorch fallback.  Arguments that
-do not go together raise ValueError.  As with any torch operator, a backward pass is captured on leaves of its own: not
-on ones that an eager graph still alive was built on (torch ties a leaf's gradient node to the stream of its first use,
-which a capture may not wait for).
+graph after one eager call) and have first-order gradients; forward-mode derivatives and tracing raise RuntimeError.
+There is no CPU or eager-PyTorch fallback.  Arguments that do not go together raise ValueError.  A backward pass is
+captured on leaves of its own (detach().requires_grad_()): with an eager graph of the same leaves alive, ending the
+capture has ended the process.
 
 The arithmetic is in csrc/sdpa.hip, ln.hip and linear.hip behind the C ABI (cg_attention_*, cg_ln_*, cg_linear_*), checks,
 memory and autograd in csrc/tokens.cpp.

@@ -620,8 +620,8 @@ int cg_gemm_timing_end(float* ms, int capacity);
 
 /*
  * s = x + r (r NULL: s = x);  y = (s - mean) / sqrt(var + eps) * weight + bias over the last axis (GAN_functions.py:35,
- * 54: norm(x + attn)).  M rows of N elements (up to 2^30), leading dimensions in elements; X, R, Y, S of `dtype`, weight and bias
- * (either may be NULL) of `wdtype`: CG_F32, or CG_BF16 where dtype is.  S (may be NULL) receives the sum, mean and rstd
+ * 54: norm(x + attn)).  M rows of N elements (up to 2^30), leading dimensions in elements; X, R, Y, S of `dtype`, weight
+ * and bias (either may be NULL) of `wdtype`: CG_F32, or CG_BF16 where dtype is.  S (may be NULL) receives the sum, mean and rstd
  * (float32, M values each; both or neither) what cg_ln_bwd needs.  Rows need only be aligned to their elements.  No
  * output overlaps an input (here and below).
  */
@@ -649,8 +649,8 @@ int cg_ln_bwd(void* dX, long long lddx, const void* dY, long long lddy, const vo
  *   words (may be NULL): B rows of (Sk + 63) / 64 64-bit words, bit j % 64 of word j / 64 set where key j of the cell is
  *     visible; cg_attention_mask_words makes them from a mask of bytes (nonzero: visible; ldm: bytes between cells)
  * A row that sees no key gives 0; one with a score of +inf or NaN, or whose visible scores are all -inf, gives NaN (the
- * softmax's own quotient); a score of -inf beside finite ones has no weight.  Whatever K and V hold at a key that `words` hides reaches no result; at a key that
- * only `causal` hides from a row, a NaN or infinity may reach that row (0 times it).  scale > 0.
+ * softmax's own quotient); a score of -inf beside finite ones has no weight.  Whatever K and V hold at a key that `words`
+ * hides reaches no result; at a key that only `causal` hides from a row, a NaN or infinity may reach that row (0 times it).  scale > 0.
  * lse2 (B, H, Sq; may be NULL): log2 of the sum of exp(s), -inf for a row that sees nothing, NaN for one whose result is;
  * cg_attention_bwd needs it.
  * workspace: cg_attention_fwd_workspace_bytes(...) bytes, 16-byte aligned (few rows and many keys: the keys are split
