@@ -6,7 +6,8 @@
 //   dx = rstd (g - mean(g) - xhat mean(g xhat)) + ds        (also the gradient of r)
 //   dw = sum over rows of dy xhat;  db = sum over rows of dy
 //
-// Bound by memory: every tensor passes once.  A row lives in the registers of its group of threads (64, 256 or 1024,
+// Bound by memory from 256 float32 columns on (2^20 rows: 5.3 TB/s), every tensor passes once; below, by the latency of a row,
+// which has a wave to itself (64 columns 1.8 TB/s, 16 0.5; bf16 256 2.7, 16 0.2).  A row lives in the registers of its group of threads (64, 256 or 1024,
 // by its length), so the mean and then the sum of squared deviations from it are two reductions over registers (no
 // cancellation of large squares).  The backward pass keeps the groups resident and walks the rows with a stride: a
 // thread owns the same columns in every row, so the column sums dw and db stay in its registers, leave as one

@@ -37,7 +37,8 @@ namespace {
 // float32 by the matrix cores.  The first product's waves go first (s_setprio), so that a SIMD's other wave is left the
 // vector unit.
 //   16 cells of 1000 to 2000 tokens, 8 heads of 64, bf16       145 us   (168 with each die holding two cells)
-//   8192 causal, 32 heads of 128, 8 of keys and values, bf16   610 us   900 TFLOP/s (633 at one priority)
+//   8192 causal, 32 heads of 128, 8 of keys and values, bf16   610 us   900 TFLOP/s (633 at one priority); 628 where what
+//                                                              rounding left is kept for the backward pass
 //   8 x 1000 tokens, 8 heads of 64, float32                    167 us    98 TFLOP/s
 // The scores of the next tile formed ahead, between this one's exponentials, gave nothing (149, 617, 173 us).
 template <typename T, int DP>
@@ -272,7 +273,9 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
 // dq of 128 rows: the forward kernel's loop with the probabilities recomputed from lse2 and ndelta as what the products
 // do v^T start from.  Three products a tile, so nearer the matrix cores' bound: 8192 causal, 32 heads of 128, 8 of keys
 // and values, bf16: 750 us, 1100 TFLOP/s; 8 x 1000 tokens, 8 heads of 64, float32: 246 us, 100 TFLOP/s.  A launch of its own
-// beside dk, dv: one launch for both would add dq up in memory, in no fixed order.
+// beside dk, dv forms s and dp twice, seven products where five would do: one launch for both would add dq up in memory, in no
+// fixed order, or keep a partial dq for every block of keys and add those (in float32 the cheaper way by its bytes: 131 MB at
+// 8 x 1000 x 8 x 64, some 55 us, against 160 for two products; not built).
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) attn_dq_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
