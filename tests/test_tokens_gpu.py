@@ -1147,3 +1147,32 @@ def test_gradients_where_one_key_has_the_weight(B, H, Hkv, Sq, Sk, D, gain):
     for what, got, ref in zip(("dq", "dk"), torch.autograd.grad(tokens.attention(*leaves), leaves, do.cuda()), refs[1:]):
         err = float((got.cpu().double() - ref).norm() / ref.norm())
         assert err <= 1.25 * 2 ** 0.5 * 2 ** -7 / 12 ** 0.5, (what, err)
+
+
+@pytest.mark.parametrize("dt", [F32, BF], ids=["float32", "bf16"])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", [(2, 4, 2, 1, 700, 64), (2, 4, 2, 16, 300, 64), (1, 2, 2, 150, 200, 128), (1, 1, 1, 1, 90, 32)])
+def test_attention_entry_points_without_the_rest_of_o(dt, B, H, Hkv, Sq, Sk, D):
+    """cg_attention_fwd and cg_attention_bwd: the same results, and gradients within the bounds that count o's rounding in
+    delta; in float32, where there is no rest, the same gradients."""
+    lib, code = _lib.load_ctypes(), 1 if dt == BF else 0
+    gen = torch.Generator().manual_seed(24)
+    cpu, (q, k, v) = make_qkv(gen, dt, B, H, Hkv, Sq, Sk, D, "dense")
+    do = rand(gen, B, Sq, H, D, dtype=dt)
+    refs, bounds = attention_reference(*cpu, do, False, None, D ** -0.5)
+    leaves, do = [t.detach().requires_grad_() for t in (q, k, v)], do.cuda()
+    want = tokens.attention(*leaves)
+    grads = torch.autograd.grad(want, leaves, do)
+    st = torch.cuda.current_stream().cuda_stream
+    at = lambda t: (t.data_ptr(), *t.stride()[:3])  # noqa: E731
+    args = (None, B, H, Hkv, Sq, Sk, D, D ** -0.5, 0, code)
+    o, lse = torch.empty_like(q), torch.empty(B, H, Sq, device="cuda")
+    dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+    n = max(lib.cg_attention_fwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, code), lib.cg_attention_bwd_workspace_bytes(B, H, Hkv, Sq, Sk, D, code))
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    assert lib.cg_attention_fwd(o.data_ptr(), lse.data_ptr(), *at(q), *at(k), *at(v), *args, ws.data_ptr(), n, st) == 0
+    assert lib.cg_attention_bwd(dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *at(do), o.data_ptr(), lse.data_ptr(), *at(q), *at(k), *at(v),
+                                *args, ws.data_ptr(), n, st) == 0
+    assert torch.equal(o, want)
+    for what, got, ref, b, g in zip(("dq", "dk", "dv"), (dq, dk, dv), refs[1:], bounds[1:], grads):
+        within(got, ref, b, what)
+        assert torch.equal(got, g) or dt == BF and what != "dv"

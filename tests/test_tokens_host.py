@@ -213,3 +213,18 @@ def test_workspaces_hold_what_goes_through_them(dtype):
         assert b >= B * H * Sq * 8
         split += (f > 0) + (b > B * H * Sq * 8 + 16)
     assert split >= 5
+
+
+def test_attention_entry_points_with_the_rest_of_o_refuse():
+    lib = _lib.load_ctypes()
+    st = (8 * 4 * 64, 4 * 64, 64)
+    off = C.c_void_p((1 << 20) + 8)
+
+    def fwd(low, dtype=1):
+        return lib.cg_attention_fwd_low(P, low, None, P, *st, P, *st, P, *st, None, 2, 4, 4, 8, 8, 64, 0.1, 0, dtype, None, 0, None)
+
+    def bwd(low, dtype=1):
+        return lib.cg_attention_bwd_low(P, P, P, P, *st, P, low, P, P, *st, P, *st, P, *st, None, 2, 4, 4, 8, 8, 64, 0.1, 0, dtype, None, 0, None)
+    assert fwd(P, 0) == -1 and bwd(P, 0) == -1               # float32 has no rest
+    assert fwd(off) == -2 and bwd(off) == -2
+    assert bwd(None) == -3 and bwd(P) == -3
